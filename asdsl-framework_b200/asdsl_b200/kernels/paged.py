@@ -225,12 +225,15 @@ class AttentionWorkspace:
     """Device scratch of the attention calls of ONE stream; grows to the largest call.
 
     Calls that may overlap in time (on several streams) need one each.  Grown outside graph capture
-    only: run a step once before capturing it.
+    only: run a step once before capturing it.  A captured graph goes on using the buffers that it was
+    captured with, so keep the workspace as long as the graph: buffers that a later, larger call outgrew
+    stay with it.
     """
 
     def __init__(self):
         self._ws: torch.Tensor | None = None
         self._merge: torch.Tensor | None = None
+        self._outgrown: list[torch.Tensor] = []
         self._bytes: dict[tuple, int] = {}
 
     def _grown(self, t, n: int, dtype, device, fill: bool):
@@ -238,6 +241,10 @@ class AttentionWorkspace:
             return t
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the attention workspace must grow: run the step once before capturing it")
+        if t is not None:
+            self._outgrown.append(t)
+            if t.device == device:
+                n = max(n, t.numel() + t.numel() // 2)  # what is outgrown adds up to twice the buffer in use at most
         return (torch.zeros if fill else torch.empty)(n, dtype=dtype, device=device)
 
     def _size(self, device, entry: str, *key) -> int:

@@ -1,0 +1,51 @@
+"""The batch operators where a user meets their edges.  References and bounds are those of test_batch_gpu
+(64 bits, derived there from the formulas)."""
+
+import pytest
+import torch
+
+from test_batch_gpu import BF, _batch, _gen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kernels(native):
+    import asdsl_b200.kernels as k
+
+    return k
+
+
+def test_graph_outlives_workspace_growth(kernels):
+    """A captured decode step replays the same bits after larger calls have grown its workspace, and leaves memory that
+    was allocated since alone."""
+    lens = [9000, 70, 4000]
+    q, cache, table, lens_t, _, _ = _batch(kernels, lens, [1, 1, 1], 6, 2, 64, 16, BF, BF)
+    pages = table[0, :200].contiguous()
+    ws = kernels.AttentionWorkspace()
+
+    def step():
+        return (*kernels.attention_paged(q, cache, table, lens_t, return_lse=True, workspace=ws),
+                *kernels.attention_shared_prefix(q, cache, pages, 3200, table, lens_t, return_lse=True, workspace=ws))
+
+    want = [t.clone() for t in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    # many more requests and rows than before, on the same workspace
+    n, m = 9000, 2
+    many = torch.randn(n * m, 6, 64, device="cuda", generator=_gen(1)).to(BF)
+    wide, long = table[:1].expand(n, -1), lens_t[:1].expand(n).contiguous()
+    cu = torch.arange(0, n * m + 1, m, dtype=torch.int32, device="cuda")
+    big = kernels.attention_paged(many, cache, wide[:, :4], long.clamp(max=64), cu, workspace=ws).clone()
+    kernels.attention_shared_prefix(many, cache, pages, 64, wide[:, :4], long.clamp(max=64), cu, workspace=ws)
+    # whatever the allocator has free now is taken and filled
+    fill = [torch.full((1 << 20,), 0x5A5A5A5A, dtype=torch.int32, device="cuda") for _ in range(64)]
+    for _ in range(3):
+        for t in got:
+            t.fill_(7)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        again = kernels.attention_paged(many, cache, wide[:, :4], long.clamp(max=64), cu, workspace=ws)
+        assert torch.equal(again, big)
+    assert all((t == 0x5A5A5A5A).all() for t in fill)
