@@ -225,9 +225,10 @@ class AttentionWorkspace:
     """Device scratch of the attention calls of ONE stream; grows to the largest call.
 
     Calls that may overlap in time (on several streams) need one each.  Grown outside graph capture
-    only: run a step once before capturing it.  A captured graph goes on using the buffers that it was
+    only: run a step once on it before capturing one.  A captured graph goes on using the buffers that it was
     captured with, so keep the workspace as long as the graph: buffers that a later, larger call outgrew
-    stay with it.
+    stay with it.  A captured call that brings no workspace takes its scratch from the graph's own memory
+    (one more small launch, which clears the arrival counters).
     """
 
     def __init__(self):
@@ -268,11 +269,30 @@ class AttentionWorkspace:
         return self._merge
 
 
+class _CaptureWorkspace(AttentionWorkspace):
+    """Scratch of one captured call, from the graph's own pool: it lives as long as the graph and is no other
+    call's.  The arrival counters are cleared by the graph."""
+
+    def sized(self, device, n_req: int, tokens: int, heads: int, kv_heads: int) -> torch.Tensor:
+        n = self._size(device, "asdsl_b200_attention_workspace_bytes", n_req, tokens, heads, kv_heads)
+        counters = self._size(device, "asdsl_b200_attention_workspace_bytes", 0, 0, heads, kv_heads)  # their offset
+        ws = torch.empty(n, dtype=torch.uint8, device=device)
+        ws[counters:].zero_()
+        return ws
+
+    def merge(self, device, tokens: int, heads: int, dim: int) -> torch.Tensor:
+        n = self._size(device, "asdsl_b200_attention_merge_bytes", tokens, heads, dim)
+        return torch.empty(n, dtype=torch.uint8, device=device)
+
+
 _stream_workspaces: dict[tuple, AttentionWorkspace] = {}
+_capture_workspace = _CaptureWorkspace()  # holds sizes, no buffers
 
 
 def _workspace(device) -> AttentionWorkspace:
     """The workspace of torch's current stream, kept for calls that bring none."""
+    if torch.cuda.is_current_stream_capturing():
+        return _capture_workspace
     key = (device.index, _raw_stream(device.index))
     ws = _stream_workspaces.get(key)
     if ws is None:

@@ -49,3 +49,26 @@ def test_graph_outlives_workspace_growth(kernels):
         again = kernels.attention_paged(many, cache, wide[:, :4], long.clamp(max=64), cu, workspace=ws)
         assert torch.equal(again, big)
     assert all((t == 0x5A5A5A5A).all() for t in fill)
+
+
+@pytest.mark.parametrize("prefix", [False, True])
+def test_capture_without_a_workspace(kernels, prefix):
+    """A call that brings no workspace can be captured, and the graph keeps what it needs whatever is called after it."""
+    lens, news = [3000, 70, 400], [1, 40, 2]
+    q, cache, table, lens_t, cu, _ = _batch(kernels, lens, news, 6, 2, 64, 16, BF, BF)
+    pages = table[0, :4].contiguous()
+
+    def step():
+        if prefix:
+            return kernels.attention_shared_prefix(q, cache, pages, 64, table, lens_t, cu, return_lse=True)
+        return kernels.attention_paged(q, cache, table, lens_t, cu, return_lse=True)
+
+    want = [t.clone() for t in step()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = step()
+    for _ in range(3):
+        out.fill_(7), lse.fill_(7)
+        graph.replay()
+        step()  # eagerly between replays
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
