@@ -286,6 +286,7 @@ class _CaptureWorkspace(AttentionWorkspace):
 
 
 _stream_workspaces: dict[tuple, AttentionWorkspace] = {}
+_MAX_STREAM_WORKSPACES = 16  # about 30 MB each; the oldest goes, in its stream's order, and is made anew when wanted
 _capture_workspace = _CaptureWorkspace()  # holds sizes, no buffers
 
 
@@ -296,6 +297,8 @@ def _workspace(device) -> AttentionWorkspace:
     key = (device.index, _raw_stream(device.index))
     ws = _stream_workspaces.get(key)
     if ws is None:
+        if len(_stream_workspaces) >= _MAX_STREAM_WORKSPACES:
+            del _stream_workspaces[next(iter(_stream_workspaces))]
         ws = _stream_workspaces[key] = AttentionWorkspace()
     return ws
 

@@ -34,3 +34,16 @@ def test_workspace_growth_adds_up(workspace):
         ws = workspace.sized(cpu, n, n, 1, 1)
     held = sum(t.numel() for t in workspace._outgrown)
     assert ws.numel() >= 20990 and held <= 2 * ws.numel()
+
+
+def test_stream_workspaces_are_bounded(monkeypatch):
+    """Streams that come and go do not each keep a workspace for good; a stream in use keeps its own."""
+    from asdsl_b200.kernels import paged
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(paged, "_stream_workspaces", {})
+    for stream in range(200):
+        monkeypatch.setattr(paged, "_raw_stream", lambda index, s=stream: s)
+        ws = paged._workspace(torch.device("cuda", 0))
+        assert paged._workspace(torch.device("cuda", 0)) is ws
+    assert len(paged._stream_workspaces) <= 32
