@@ -94,6 +94,9 @@ class StepPlan:
     left.  The rest is rewritten by each ``plan_step`` of n requests: ``cu_q`` [n + 1], ``total_lens``
     [n], and ``slots``, ``positions``, ``requests`` [max_tokens] of the new tokens (-1, 0, -1 past the
     last), ``counts`` = (pages taken, new tokens, flags).
+
+    ``total_lens`` may be the next step's kv_lens: a step that reads it writes its totals to another buffer,
+    which ``total_lens`` then names.
     """
 
     FREE_SHORT, TABLE_NARROW, TOKENS_OVER = 1, 2, 4  # counts[2]
@@ -107,19 +110,20 @@ class StepPlan:
         self.page_size, self.max_tokens = page_size, max_tokens
         self._table = torch.full((max_requests, max_pages), -1, dtype=torch.int32, device=device)
         self._cu = torch.zeros(max_requests + 1, dtype=torch.int32, device=device)
-        self._total = torch.zeros(max_requests, dtype=torch.int32, device=device)
+        self._totals = torch.zeros(2, max_requests, dtype=torch.int32, device=device)
         self.slots = torch.full((max_tokens,), -1, dtype=torch.int32, device=device)
         self.positions = torch.zeros(max_tokens, dtype=torch.int32, device=device)
         self.requests = torch.full((max_tokens,), -1, dtype=torch.int32, device=device)
         self.counts = torch.zeros(3, dtype=torch.int32, device=device)
-        self._buffers = (self._table.data_ptr(), self._table.stride(0), max_pages, self._cu.data_ptr(), self._total.data_ptr(),
-                         self.slots.data_ptr(), self.positions.data_ptr(), self.requests.data_ptr(), max_tokens,
-                         self.counts.data_ptr())
-        self._set(max_requests)
+        self._total_ptrs = self._totals[0].data_ptr(), self._totals[1].data_ptr()
+        self._buffers = tuple((self._table.data_ptr(), self._table.stride(0), max_pages, self._cu.data_ptr(), total,
+                               self.slots.data_ptr(), self.positions.data_ptr(), self.requests.data_ptr(), max_tokens,
+                               self.counts.data_ptr()) for total in self._total_ptrs)
+        self._set(max_requests, 0)
 
-    def _set(self, n: int) -> None:
-        self.n = n
-        self.block_table, self.cu_q, self.total_lens = self._table[:n], self._cu[: n + 1], self._total[:n]
+    def _set(self, n: int, which: int) -> None:
+        self.n, self._which = n, which
+        self.block_table, self.cu_q, self.total_lens = self._table[:n], self._cu[: n + 1], self._totals[which, :n]
 
 
 def plan_step(plan: StepPlan, kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor) -> StepPlan:
@@ -128,7 +132,8 @@ def plan_step(plan: StepPlan, kv_lens: torch.Tensor, new_lens: torch.Tensor, fre
     The pages a request gains come from the front of `free_pages` in request order (``counts[0]`` of
     them in all).  Lengths, tables and slots stay on the device; the flags in ``counts[2]`` tell of a
     free list that was too short, a request past max_pages, or tokens past max_tokens -- what did not
-    fit has page and slot -1, which ``kv_write`` and the attention pass over.
+    fit has page and slot -1, which ``kv_write`` and the attention pass over.  kv_lens may be the last
+    step's ``plan.total_lens``; otherwise the inputs must not share memory with the plan's buffers.
     """
     table = plan._table
     device = table.device
@@ -138,10 +143,13 @@ def plan_step(plan: StepPlan, kv_lens: torch.Tensor, new_lens: torch.Tensor, fre
     _vector(free_pages, "free_pages", -1, device)
     if n > table.shape[0]:
         raise ValueError(f"{n} requests, the plan has rows for {table.shape[0]}")
-    if plan.n != n:
-        plan._set(n)
-    _call(device, "asdsl_b200_plan_step", kv_lens.data_ptr(), new_lens.data_ptr(), n, free_pages.data_ptr(),
-          free_pages.numel(), plan.page_size, *plan._buffers)
+    kv = kv_lens.data_ptr()
+    first, second = plan._total_ptrs
+    which = 1 if first <= kv < second else 0  # the totals of the last step may be read here
+    if plan.n != n or plan._which != which:
+        plan._set(n, which)
+    _call(device, "asdsl_b200_plan_step", kv, new_lens.data_ptr(), n, free_pages.data_ptr(), free_pages.numel(),
+          plan.page_size, *plan._buffers[which])
     return plan
 
 

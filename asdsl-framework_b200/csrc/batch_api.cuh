@@ -326,6 +326,18 @@ int asdsl_b200_plan_step(const int32_t* kv_lens, const int32_t* new_lens, int n_
         (n_requests > 0 && table_width > 0 && !block_table) || (n_free > 0 && !free_pages) ||
         (max_tokens > 0 && (!slots || !positions || !requests)))
         return set_error(kEinval, "plan_step: null pointer");
+    // every CTA reads the inputs for as long as it runs, whatever the others have written
+    const auto shared = [&](const void* out, long long out_n) {
+        const auto meets = [&](const void* in, long long in_n) {
+            const uintptr_t x = reinterpret_cast<uintptr_t>(in), y = reinterpret_cast<uintptr_t>(out);
+            return in_n > 0 && out_n > 0 && x < y + static_cast<uintptr_t>(out_n) * 4 && y < x + static_cast<uintptr_t>(in_n) * 4;
+        };
+        return meets(kv_lens, n_requests) || meets(new_lens, n_requests) || meets(free_pages, n_free);
+    };
+    if (shared(block_table, n_requests > 0 && table_width > 0 ? (n_requests - 1) * table_stride + table_width : 0) ||
+        shared(cu_q, n_requests + 1) || shared(total_lens, n_requests) || shared(slots, max_tokens) ||
+        shared(positions, max_tokens) || shared(requests, max_tokens) || shared(counts, 3))
+        return set_error(kEinval, "plan_step: the lengths and free_pages must not overlap what the step writes");
     PlanArgs a;
     a.kv_lens = kv_lens;
     a.new_lens = new_lens;

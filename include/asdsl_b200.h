@@ -549,7 +549,9 @@ typedef struct asdsl_b200_paged_cache {
  * of the new tokens, total_lens[n] = kv + new, and for each new token t < max_tokens its slot, position
  * and request (past the last token: -1, 0, -1).  counts[0] = pages the step takes from free_pages,
  * counts[1] = new tokens, counts[2] = flags: 1 free_pages too short (cells and slots without a page are
- * -1), 2 a request outgrew table_width (slots past it are -1), 4 more tokens than max_tokens. */
+ * -1), 2 a request outgrew table_width (slots past it are -1), 4 more tokens than max_tokens.
+ * kv_lens, new_lens and free_pages must not overlap anything that is written (total_lens of one step can be
+ * kv_lens of the next, written to a second buffer): ASDSL_B200_EINVAL. */
 int asdsl_b200_plan_step(const int32_t* kv_lens, const int32_t* new_lens, int n_requests, const int32_t* free_pages,
                          int n_free, int page_size, int32_t* block_table, long long table_stride, int table_width,
                          int32_t* cu_q, int32_t* total_lens, int32_t* slots, int32_t* positions, int32_t* requests,

@@ -1,10 +1,11 @@
 """The batch operators where a user meets their edges.  References and bounds are those of test_batch_gpu
 (64 bits, derived there from the formulas)."""
 
+import numpy as np
 import pytest
 import torch
 
-from test_batch_gpu import BF, _batch, _gen
+from test_batch_gpu import BF, _batch, _cu, _gen, _plan_by_hand
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +73,27 @@ def test_capture_without_a_workspace(kernels, prefix):
         graph.replay()
         step()  # eagerly between replays
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@pytest.mark.parametrize("n,page,new_max,tokens", [(3, 16, 1, 3), (40, 16, 30, 1200), (700, 64, 200, 140000), (1, 1, 5, 8)])
+def test_plan_fed_with_its_own_totals(kernels, n, page, new_max, tokens):
+    """A step's total_lens as the next step's kv_lens, over page boundaries and with many CTAs."""
+    r = np.random.default_rng(n)
+    kv, width = [0] * n, 2 + 8 * new_max // page
+    table = [[-1] * width for _ in range(n)]
+    plan = kernels.StepPlan(n, tokens, width, page)
+    lens = _cu(kv)
+    for step in range(8):
+        new = r.integers(0, new_max + 1, n).tolist()
+        free = (r.permutation(n * width) + step * n * width).tolist()
+        want = _plan_by_hand(kv, new, free, table, page, width, tokens)
+        kernels.plan_step(plan, lens, _cu(new), _cu(free))
+        got = (plan.block_table, plan.cu_q, plan.total_lens, plan.slots, plan.positions, plan.requests, plan.counts)
+        for name, g, w in zip(("table", "cu", "total", "slots", "positions", "requests", "counts"), got, want):
+            assert g.tolist() == w, (step, name)
+        kv, table, lens = want[2], want[0], plan.total_lens
+        if step == 5 and n > 2:
+            n -= 1  # the last request leaves
+            kv, table, lens = kv[:n], table[:n], lens[:n]
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.plan_step(plan, lens, plan.cu_q[:n], _cu(free))

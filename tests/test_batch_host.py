@@ -4,6 +4,32 @@ import pytest
 import torch
 
 
+@pytest.fixture(scope="module")
+def lib():
+    from asdsl_b200 import _lib
+    from asdsl_b200.build import build_library
+
+    build_library()
+    return _lib
+
+
+def test_plan_step_refuses_inputs_that_it_would_overwrite(lib):
+    """CTAs read the inputs while another writes the outputs, so the two must be apart (checked before any launch)."""
+    # three requests, four free pages, a table [3][2], four tokens; addresses far apart
+    at = dict(kv=0x1000, new=0x2000, free=0x3000, table=0x4000, cu=0x5000, total=0x6000, slots=0x7000, pos=0x8000, req=0x9000,
+              counts=0xA000)
+
+    def step(**kw):
+        a = {**at, **kw}
+        lib.call("asdsl_b200_plan_step", a["kv"], a["new"], 3, a["free"], 4, 16, a["table"], 2, 2, a["cu"], a["total"], a["slots"],
+                 a["pos"], a["req"], 4, a["counts"], None)
+
+    for kw in (dict(kv=at["total"]), dict(kv=at["total"] + 8), dict(new=at["total"]), dict(new=at["cu"] + 12), dict(free=at["slots"]),
+               dict(kv=at["table"] + 20), dict(kv=at["pos"] - 8), dict(new=at["req"] + 12), dict(free=at["counts"] + 8)):
+        with pytest.raises(ValueError, match="overlap"):
+            step(**kw)
+
+
 @pytest.fixture
 def workspace(monkeypatch):
     """An AttentionWorkspace on the CPU whose sizes are the calls' tokens in bytes."""
