@@ -92,14 +92,13 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan_step(const PlanArgs a) {
     int32_t* cu = plan_smem;              // [n + 1]
     int32_t* po = plan_smem + a.n + 1;    // [n + 1]
     __shared__ int warp_tok[kPlanThreads / 32], warp_pg[kPlanThreads / 32];
-    __shared__ int narrow;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         cu[0] = 0;
         po[0] = 0;
-        narrow = 0;
     }
     int tok_base = 0, pg_base = 0;
+    bool outgrown = false;
     for (int r0 = 0; r0 < a.n; r0 += kPlanThreads) {
         const int r = r0 + tid;
         int tok = 0, pg = 0;
@@ -110,7 +109,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan_step(const PlanArgs a) {
             pg = pages_for(total, a) - pages_for(kv, a);
             if (blockIdx.x == 0) {
                 a.total[r] = total;
-                if (tok > 0 && a.page.div(total - 1) >= a.width) narrow = 1;
+                if (tok > 0 && a.page.div(total - 1) >= a.width) outgrown = true;
             }
         }
 #pragma unroll
@@ -144,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_plan_step(const PlanArgs a) {
         pg_base = pa;
         __syncthreads();
     }
-    __syncthreads();
+    const bool narrow = __syncthreads_or(outgrown);
     const int total_tok = tok_base, total_pg = pg_base;
     if (blockIdx.x == 0) {
         for (int r = tid; r <= a.n; r += kPlanThreads) a.cu[r] = cu[r];

@@ -97,3 +97,17 @@ def test_plan_fed_with_its_own_totals(kernels, n, page, new_max, tokens):
             kv, table, lens = kv[:n], table[:n], lens[:n]
     with pytest.raises(ValueError, match="overlap"):
         kernels.plan_step(plan, lens, plan.cu_q[:n], _cu(free))
+
+
+def test_plan_flags_one_request_that_outgrows_the_table(kernels):
+    """The flag comes from whichever thread meets the request, the same in every launch."""
+    plan = kernels.StepPlan(900, 900, 2, 16)
+    new, free = _cu([1] * 900), _cu(list(range(2000)))
+    for b in (0, 31, 511, 512, 899):
+        kv = torch.zeros(900, dtype=torch.int32, device="cuda")
+        kernels.plan_step(plan, kv, new, free)
+        assert plan.counts.tolist() == [900, 900, 0]
+        kv[b] = 32
+        for _ in range(20):
+            kernels.plan_step(plan, kv, new, free)
+            assert plan.counts.tolist() == [899, 900, 2]
