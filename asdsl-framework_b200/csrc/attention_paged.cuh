@@ -54,6 +54,7 @@ constexpr float kLn2 = 0.693147180559945309f;
 // ---- one request's share -------------------------------------------------------------------
 struct ReqRows {
     int first, n, len;  // first row in q, rows (tokens), keys
+    int held;           // of those keys, what the table has cells for: the others are unseen
 };
 
 __device__ __forceinline__ ReqRows request_rows(const AttnPagedArgs& a, int b) {
@@ -70,8 +71,8 @@ __device__ __forceinline__ ReqRows request_rows(const AttnPagedArgs& a, int b) {
         r.n = b < a.tokens ? 1 : 0;
     }
     const long long cap = static_cast<long long>(a.width) * a.c.page.d;
-    const int len = max(a.lens ? a.lens[b] : a.const_len, 0);
-    r.len = len < cap ? len : static_cast<int>(cap);
+    r.len = max(a.lens ? a.lens[b] : a.const_len, 0);
+    r.held = r.len < cap ? r.len : static_cast<int>(cap);
     return r;
 }
 
@@ -81,13 +82,16 @@ struct KeySpan {
     __device__ __forceinline__ int key(int u) const { return u < sunk ? u : lo + (u - sunk); }
 };
 
+// first key of the window of a row at position p (p + 1 - window would leave 32 bits for rows before key 0)
+__device__ __forceinline__ int window_low(const AttnPagedArgs& a, int p) { return p < a.window ? 0 : p - a.window + 1; }
+
 __device__ __forceinline__ KeySpan key_span(const AttnPagedArgs& a, const ReqRows& r, int i0, int i1) {
-    KeySpan s{0, 0, r.len};
+    KeySpan s{0, 0, r.held};
     if (a.causal) {
-        const int hi = min(max(r.len - r.n + i1, 0), r.len);
+        const int hi = min(max(r.len - r.n + i1, 0), r.held);
         s.n = hi;
         if (a.window > 0) {
-            s.lo = min(max(r.len - r.n + i0 - a.window + 1, 0), hi);
+            s.lo = min(window_low(a, r.len - r.n + i0), hi);
             s.sunk = min(a.sinks, s.lo);
             s.n = s.sunk + hi - s.lo;
         }
@@ -96,7 +100,7 @@ __device__ __forceinline__ KeySpan key_span(const AttnPagedArgs& a, const ReqRow
 }
 
 __device__ __forceinline__ bool row_sees(const AttnPagedArgs& a, int p, int j) {
-    return j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks);
+    return j <= p && (a.window <= 0 || j >= window_low(a, p) || j < a.sinks);
 }
 
 // ---- 16-bit tensor-core product ------------------------------------------------------------

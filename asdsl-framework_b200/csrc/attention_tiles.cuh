@@ -565,8 +565,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attention_tiles_paged(const
                 u_high = p < 0 ? -1 : p + shift;
                 t_high = p_first < 0 ? -1 : p_first + shift;
                 if (a.window > 0) {
-                    u_low = max(p - a.window + 1 + shift, 0);
-                    t_low = max(p_last - a.window + 1 + shift, 0);
+                    u_low = max(window_low(a, p) + shift, 0);
+                    t_low = max(window_low(a, p_last) + shift, 0);
                     u_sink = a.sinks;
                 }
             }

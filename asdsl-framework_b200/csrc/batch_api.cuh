@@ -427,8 +427,7 @@ int asdsl_b200_attention_paged(const void* q, int q_dtype, long long q_token_str
                                 workspace, workspace_bytes))
         return rc;
     if (n_tokens == 0 || n_requests == 0) return kOk;
-    // a window that reaches every key is none
-    a.window = window < static_cast<long long>(table_width) * cache->page_size ? window : 0;
+    a.window = window;
     a.sinks = sinks;
     float* rows_ws = reinterpret_cast<float*>(static_cast<char*>(workspace) + attention_part_bytes());
     return launch_attention(a, q_dtype, cache->dtype, cache->head_dim, rows_ws, nullptr, static_cast<cudaStream_t>(stream));

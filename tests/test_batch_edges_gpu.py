@@ -1,11 +1,13 @@
 """The batch operators where a user meets their edges.  References and bounds are those of test_batch_gpu
 (64 bits, derived there from the formulas)."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
 
-from test_batch_gpu import BF, _batch, _cu, _gen, _plan_by_hand
+from test_batch_gpu import BF, I8, _batch, _check, _cu, _dense, _fast_reference, _gen, _plan_by_hand
 
 pytestmark = pytest.mark.gpu
 
@@ -111,3 +113,27 @@ def test_plan_flags_one_request_that_outgrows_the_table(kernels):
         for _ in range(20):
             kernels.plan_step(plan, kv, new, free)
             assert plan.counts.tolist() == [899, 900, 2]
+
+
+@pytest.mark.parametrize("m,window,sinks", [(1, 50, 0), (1, 36, 0), (1, 30, 2), (4, 0, 0), (4, 60, 3), (60, 0, 0), (60, 45, 2), (60, 100, 0)])
+@pytest.mark.parametrize("cache_dtype", [BF, I8])
+def test_attention_table_narrower_than_the_lengths(kernels, m, window, sinks, cache_dtype):
+    """Positions come from kv_lens; keys past the table's last page are unseen."""
+    q, cache, table, lens_t, cu, _ = _batch(kernels, [100, 50], [m, m], 6, 2, 128, 16, BF, cache_dtype, with_cu=True)
+    table = table[:, :4].contiguous()  # 64 positions
+    out, lse = kernels.attention_paged(q, cache, table, lens_t, cu, window=window, sinks=sinks, return_lse=True)
+    want = []
+    for b, n in enumerate((100, 50)):
+        k, v = _dense(cache, table[b, : -(-min(n, 64) // 16)], min(n, 64))
+        want.append(_fast_reference(q[b * m : b * m + m].double(), k, v, n - m, window, sinks, 1 / math.sqrt(128)))
+    _check(out, lse, tuple(torch.cat(x) for x in zip(*want)), BF)
+
+
+@pytest.mark.parametrize("m", [1, 60])
+def test_attention_windows_of_any_size(kernels, m):
+    """The largest windows and sinks with more rows than keys (positions before key 0) stay within 32 bits."""
+    q, cache, table, lens_t, cu, _ = _batch(kernels, [40, 3], [m, m], 6, 2, 64, 16, BF, BF, with_cu=True)
+    want = kernels.attention_paged(q, cache, table, lens_t, cu, return_lse=True)
+    for window, sinks in ((2**31 - 1, 0), (2**31 - 1, 2**31 - 1), (2**31 - 30, 5), (1, 2**31 - 1)):
+        got = kernels.attention_paged(q, cache, table, lens_t, cu, window=window, sinks=sinks, return_lse=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (window, sinks)
