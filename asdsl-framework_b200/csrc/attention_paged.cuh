@@ -45,8 +45,7 @@ struct AttnPagedArgs {
     FastDiv by_group;
     int small_rows;           // requests with up to this many rows (tokens x group) go to the few-rows kernel
     float* part;              // partial results of keys split over CTAs
-    unsigned int* count;      // [n_units] arrivals per unit, zero before and after a launch
-    long long n_units;
+    unsigned int* count;      // [n_req][kv_heads] arrivals per unit, zero before and after a launch
 };
 
 constexpr float kLn2 = 0.693147180559945309f;
@@ -224,11 +223,11 @@ constexpr int kRowsMaxCtas = 4;
 __host__ __device__ constexpr int part_floats(int rows, int D) { return rows * (D + 2); }
 
 // ---- the few-rows kernel -------------------------------------------------------------------
-// A unit is 8 NR query rows (group heads of a KV head times tokens) of one request and KV head; its keys
-// come in iterations of 16 to each warp (6 for 16-bit pages, 8 for int8), which keep their own maximum, sum and output.  All
-// units' iterations form one line that is cut into equal runs, one per CTA, so the work is even whatever
-// the requests' lengths; a unit cut by a run's end leaves (max, sum, output) partials that the last CTA to
-// arrive merges in CTA order (same bits every time).
+// A unit is a request and KV head: the query rows (group heads times tokens) are one tile of up to 8 NR, which
+// the launch rule sees to.  Its keys come in iterations of 16 to each of the 4 warps, which keep their own
+// maximum, sum and output.  All units' iterations form one line that is cut into equal runs, one per CTA, so
+// the work is even whatever the requests' lengths; a unit cut by a run's end leaves (max, sum, output)
+// partials that the last CTA to arrive merges in CTA order (same bits every time).
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that the 16-high side of the
 // tensor-core tile is keys (then dims) and the 8-wide side the few rows: half the products, registers and
@@ -237,7 +236,7 @@ __host__ __device__ constexpr int part_floats(int rows, int D) { return rows * (
 // transpose per 8 keys.
 //
 // Bound by the cache's bytes.  A warp copies whole 128-byte lines of its keys, with cp.async, into its own
-// ring in shared memory (16 KB in flight per warp, no block-wide barriers) and reads them back as operand
+// ring in shared memory (16 KB in flight per warp, 8 KB for int8; no block-wide barriers) and reads them back as operand
 // fragments: the contraction index of S and the dims of O are permuted so that a lane's fragments are
 // 16 consecutive bytes of a key's row.  Copies of 64-byte half lines, each lane its own fragments, had
 // the L2's tag lookups at 61 % and held the kernel at 4.5 TB/s.
@@ -248,20 +247,17 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
     constexpr int NK = G::kRow / 64;    // 16-byte K pieces per lane and key
     constexpr int kLanes = G::kRow < 128 ? 4 : 8, kGroup = 32 / kLanes;  // lanes of a row, rows of a copy
     constexpr int ES = I8 ? 1 : 2;
-    constexpr int R = 8 * NR;           // rows of a unit
     using C = std::conditional_t<I8, __half, T>;  // operand type of the products
     extern __shared__ __align__(128) uint8_t rows_smem[];
     __shared__ long long s_scan[2][G::kWarps], s_base;
-    __shared__ int s_unit[G::kWarps], s_req, s_unit_base, s_last;
+    __shared__ int s_req, s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
     const int kv_heads = a.c.kv_heads;
 
-    auto tiles_of = [&](const ReqRows& r) { return r.n * a.group <= a.small_rows ? (r.n * a.group + R - 1) / R : 0; };
-    auto iters_of = [&](const ReqRows& r, int tiles) {
-        if (tiles == 0) return 0;
-        int n = key_span(a, r, 0, r.n).n;
-        if (tiles > 1 && a.causal && a.window > 0) n = min(n, a.sinks + a.window + R / a.group + 2);
-        return max((n + G::kTile - 1) / G::kTile, 1);
+    // iterations of a request's units (0: no rows, or more than this kernel takes)
+    auto iters_of = [&](const ReqRows& r) {
+        const int rows = r.n * a.group;
+        return rows == 0 || rows > a.small_rows ? 0 : max((key_span(a, r, 0, r.n).n + G::kTile - 1) / G::kTile, 1);
     };
     // The length of the line, in iterations and in chunks; then the request of this CTA's first chunk.  A
     // second pass over the requests is needed only where there are more of them than threads.
@@ -270,47 +266,33 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
     const bool once = a.n_req <= G::kThreads;
     for (int pass = 0; pass < 2; ++pass) {
         long long base[2] = {0, 0};
-        int unit_base = 0;
         for (int r0 = 0; r0 < a.n_req; r0 += G::kThreads) {
-            int units = 0, iters = 0;
-            if (r0 + tid < a.n_req) {
-                const ReqRows r = request_rows(a, r0 + tid);
-                const int tiles = tiles_of(r);
-                iters = iters_of(r, tiles);
-                units = tiles * kv_heads;
-            }
-            const long long cnt[2] = {static_cast<long long>(units) * iters,
-                                      static_cast<long long>(units) * (iters <= kRowsWhole ? 1 : (iters + 1) / 2)};
+            const int iters = r0 + tid < a.n_req ? iters_of(request_rows(a, r0 + tid)) : 0;
+            const long long cnt[2] = {static_cast<long long>(kv_heads) * iters,
+                                      static_cast<long long>(kv_heads) * (iters <= kRowsWhole ? min(iters, 1) : (iters + 1) / 2)};
             long long inc[2] = {cnt[0], cnt[1]};
-            int uinc = units;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long t0 = __shfl_up_sync(0xffffffffu, inc[0], o), t1 = __shfl_up_sync(0xffffffffu, inc[1], o);
-                const int u = __shfl_up_sync(0xffffffffu, uinc, o);
                 if (lane >= o) {
                     inc[0] += t0;
                     inc[1] += t1;
-                    uinc += u;
                 }
             }
             if (lane == 31) {
                 s_scan[0][warp] = inc[0];
                 s_scan[1][warp] = inc[1];
-                s_unit[warp] = uinc;
             }
             __syncthreads();
             long long before[2] = {base[0], base[1]};
-            int ubefore = unit_base;
 #pragma unroll
             for (int w = 0; w < G::kWarps; ++w) {
                 if (w < warp) {
                     before[0] += s_scan[0][w];
                     before[1] += s_scan[1][w];
-                    ubefore += s_unit[w];
                 }
                 base[0] += s_scan[0][w];
                 base[1] += s_scan[1][w];
-                unit_base += s_unit[w];
             }
             if (once) {
                 chunk = base[0] < static_cast<long long>(kRowsLong) * gridDim.x ? 2 : 1;
@@ -324,7 +306,6 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
                 if (n > 0 && mine <= begin && begin < mine + n) {
                     s_req = r0 + tid;
                     s_base = mine;
-                    s_unit_base = ubefore + uinc - units;
                 }
             }
             __syncthreads();
@@ -339,9 +320,9 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
             if (once) break;
         }
     }
-    int req = s_req, unit_base = s_unit_base;
+    int req = s_req;
     long long req_base = s_base;
-    auto chunks_of = [&](int iters) { return chunk == 1 ? iters : (iters <= kRowsWhole ? 1 : (iters + 1) / 2); };
+    auto chunks_of = [&](int iters) { return chunk == 1 ? iters : (iters <= kRowsWhole ? min(iters, 1) : (iters + 1) / 2); };
     auto start_of = [&](int cta) { return total * cta / active; };
     auto cta_of = [&](long long y) { return static_cast<int>(((y + 1) * active - 1) / total); };  // last with start <= y
 
@@ -349,25 +330,21 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
                    haves = offs + G::kOffsets;  // per stage: which of its 16 keys exist
     for (long long x = begin; x < end;) {
         ReqRows r = request_rows(a, req);
-        int tiles = tiles_of(r), iters = iters_of(r, tiles), chunks = chunks_of(iters);
-        while (x >= req_base + static_cast<long long>(tiles) * kv_heads * chunks) {
-            req_base += static_cast<long long>(tiles) * kv_heads * chunks;
-            unit_base += tiles * kv_heads;
+        int iters = iters_of(r), chunks = chunks_of(iters);
+        while (x >= req_base + static_cast<long long>(kv_heads) * chunks) {
+            req_base += static_cast<long long>(kv_heads) * chunks;
             ++req;
             r = request_rows(a, req);
-            tiles = tiles_of(r);
-            iters = iters_of(r, tiles);
+            iters = iters_of(r);
             chunks = chunks_of(iters);
         }
-        const int local = static_cast<int>((x - req_base) / chunks);
-        const long long unit_x = req_base + static_cast<long long>(local) * chunks;
-        const int h = local / tiles, row0 = (local - h * tiles) * R;
+        const int h = static_cast<int>((x - req_base) / chunks);
+        const long long unit_x = req_base + static_cast<long long>(h) * chunks;
         const int c0 = static_cast<int>(x - unit_x), c1 = static_cast<int>(min(end - unit_x, static_cast<long long>(chunks)));
         const int it0 = c0 * chunk, it1 = c1 == chunks ? iters : c1 * chunk;
-        const int rows = min(R, r.n * a.group - row0);
-        const int i0 = row0 / a.group, i1 = (row0 + rows - 1) / a.group + 1;
-        const KeySpan span = key_span(a, r, i0, i1);
-        const bool same = !a.causal || i1 - i0 == 1;  // all rows see all of the span
+        const int rows = r.n * a.group;
+        const KeySpan span = key_span(a, r, 0, r.n);
+        const bool same = !a.causal || r.n == 1;  // all rows see all of the span
 
         // page of this lane's key, of iteration `it` (lanes 0-15) or the next (16-31); -1: no such key
         const int32_t* tab = a.table + req * a.table_stride;
@@ -445,10 +422,10 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
         float q_scale[NR][2];  // log2 units of a score of rows 2 c and 2 c + 1
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            const int rr = row0 + g + 8 * n, i = rr / a.group;
-            const bool live = g + 8 * n < rows;
+            const int row = g + 8 * n, i = row / a.group;
+            const bool live = row < rows;
             const T* qp = static_cast<const T*>(a.q) + (r.first + i) * a.q_token_stride +
-                          (h * a.group + rr - i * a.group) * a.q_head_stride;
+                          (h * a.group + row - i * a.group) * a.q_head_stride;
 #pragma unroll
             for (int i2 = 0; i2 < NQ; ++i2) {
                 // 16-bit: piece i covers dims 32 i + 8 c ..; int8: 16 dims 64 (i / 2) + 16 c + 8 (i % 2)
@@ -486,7 +463,7 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = 2 * c + e + 8 * n;
-                pos[n][e] = row < rows ? r.len - r.n + (row0 + row) / a.group : -1;
+                pos[n][e] = row < rows ? r.len - r.n + row / a.group : -1;
             }
 
         float o[NR][NB][4][4];  // [.][block][w][2 k + e]: dim 64 block + 8 g + 2 w + k
@@ -739,13 +716,11 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
         // a row of the joined result: DP dims per thread, from n results of it `stride` rows apart
         constexpr int DP = 8, kPer = D / DP;
         const bool split = c0 > 0 || c1 < chunks;
-        // more units than rows allow, as of row starts that do not ascend: their rows are not written
-        const bool counted = unit_base + local < a.n_units;
         constexpr int PF = part_floats(16, D);
         float* mine = a.part + static_cast<long long>(2 * blockIdx.x + (x == begin ? 0 : 1)) * PF;
         auto store = [&](int row, int d0, float(&acc)[DP], float mx, float sum) {
-            const int rr = row0 + row, i = rr / a.group;
-            const long long qh = static_cast<long long>(r.first + i) * a.heads + h * a.group + (rr - i * a.group);
+            const int i = row / a.group;
+            const long long qh = static_cast<long long>(r.first + i) * a.heads + h * a.group + (row - i * a.group);
             attention_store<T, DP>(a, 0, qh, D, d0, d0 == 0, acc, mx, sum);
         };
         for (int row = tid / kPer; row < rows; row += G::kThreads / kPer) {
@@ -773,11 +748,11 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
             }
         }
         // ---- a unit split over CTAs: the last to arrive merges the parts in CTA order ----
-        if (split && counted) {
+        if (split) {
             const int ca = cta_of(unit_x), n = cta_of(unit_x + chunks - 1) - ca + 1;
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicInc(a.count + unit_base + local, n - 1) == static_cast<unsigned>(n - 1);
+            if (tid == 0) s_last = atomicInc(a.count + static_cast<long long>(req) * kv_heads + h, n - 1) == static_cast<unsigned>(n - 1);
             __syncthreads();
             if (s_last) {
                 __threadfence();

@@ -99,9 +99,6 @@ inline size_t attention_part_bytes() {
 }
 inline long long attention_part_rows() { return static_cast<long long>(kUnitRows) * sm_count(); }
 inline size_t attention_rows_bytes() { return static_cast<size_t>(attention_part_rows()) * (128 + 2) * sizeof(float); }
-inline long long attention_units(int n_req, int tokens, int heads, int kv_heads) {
-    return (static_cast<long long>(tokens) * (heads / kv_heads) / 8 + n_req) * kv_heads;
-}
 
 template <typename T, bool I8, int D, int NR>
 inline int launch_rows(const AttnPagedArgs& a, cudaStream_t st) {
@@ -172,7 +169,7 @@ inline int launch_attention_as(AttnPagedArgs a, float* rows_ws, AttnParts* parts
     const long long few_rows = single && keys >= kManyKeys && !one_each ? kSmallRows / 2 : kSmallRows;
     const bool only_few = one_each ? a.group <= kSmallRows : all_rows <= few_rows;
     const bool only_many = !only_few && (one_each || single);
-    a.small_rows = only_few ? 0x7fffffff : (only_many ? 0 : kSmallRows);
+    a.small_rows = only_many ? 0 : kSmallRows;
     if (!only_few) {
         // an upper bound of the 256-row blocks, and key splits while those leave SMs idle
         const long long reqs = only_many ? a.n_req : std::min<long long>(a.n_req, all_rows / (kSmallRows + 1));
@@ -303,7 +300,6 @@ inline int attention_args(const char* fn, AttnPagedArgs* a, const void* q, int q
     a->out = out;
     a->lse = lse;
     a->part = static_cast<float*>(ws);
-    a->n_units = attention_units(n_req, tokens, heads, cache->kv_heads);
     a->count = reinterpret_cast<unsigned int*>(static_cast<char*>(ws) + attention_part_bytes() + attention_rows_bytes());
     return kOk;
 }
@@ -407,7 +403,7 @@ int asdsl_b200_kv_write(const asdsl_b200_paged_cache* cache, const void* k, cons
 
 size_t asdsl_b200_attention_workspace_bytes(int n_requests, int n_tokens, int heads, int kv_heads) {
     if (n_requests < 0 || n_tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-    return attention_part_bytes() + attention_rows_bytes() + static_cast<size_t>(attention_units(n_requests, n_tokens, heads, kv_heads)) * 4;
+    return attention_part_bytes() + attention_rows_bytes() + static_cast<size_t>(n_requests) * kv_heads * sizeof(unsigned int);
 }
 
 size_t asdsl_b200_attention_merge_bytes(int n_tokens, int heads, int head_dim) {
