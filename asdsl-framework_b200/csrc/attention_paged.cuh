@@ -10,7 +10,11 @@
 //
 // in one pass over the keys, the maximum and sum in fp32; P is rounded to the query's 16-bit type for
 // the second product (half a unit in the last place of each weight, as of the output itself), the sum is of the
-// unrounded weights.
+// unrounded weights.  bf16 has fp32's range; fp16 weights are lifted by a power of two (kLift: M stands that much
+// below the maximum, which the quotient does not see), since a long tail of keys can carry the output although
+// each of its weights is far below the largest: with weights up to 1, those below 2^-14 of it lost bits and those
+// below 2^-25 counted in the sum alone.  Lifted, a weight keeps all its bits down to 2^-29 of the largest (int8
+// pages: 2^-28, times its V scale over the block's largest so far; the many-rows kernel 2^-26 and 2^-25).
 #pragma once
 
 #include <type_traits>
@@ -248,6 +252,8 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
     constexpr int kLanes = G::kRow < 128 ? 4 : 8, kGroup = 32 / kLanes;  // lanes of a row, rows of a copy
     constexpr int ES = I8 ? 1 : 2;
     using C = std::conditional_t<I8, __half, T>;  // operand type of the products
+    // log2 of the largest weight: below fp16's 65504 (int8: times a V scale over its unit, below 2)
+    constexpr float kLift = !std::is_same<C, __half>::value ? 0.0f : (I8 ? 14.0f : 15.0f);
     extern __shared__ __align__(128) uint8_t rows_smem[];
     __shared__ long long s_scan[2][G::kWarps], s_base;
     __shared__ int s_req, s_last;
@@ -467,7 +473,7 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
             }
 
         float o[NR][NB][4][4];  // [.][block][w][2 k + e]: dim 64 block + 8 g + 2 w + k
-        float m[NR][2], l[NR][2];
+        float m[NR][2], l[NR][2];  // m: the running maximum less kLift
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
             m[n][0] = m[n][1] = -INFINITY;
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
                     for (int e = 0; e < 2; ++e) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], sh));
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float mn = fmaxf(m[n][e], mx[e] * q_scale[n][e]);
+                    const float mn = fmaxf(m[n][e], fmaf(mx[e], q_scale[n][e], -kLift));
                     const float base = mn == -INFINITY ? 0.0f : mn;
                     al[e] = ex2(m[n][e] - base);
                     m[n][e] = mn;

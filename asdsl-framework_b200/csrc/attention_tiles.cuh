@@ -10,9 +10,9 @@
 //
 // While one tile's softmax runs, the tensor cores work on the other tile.  P overwrites S in place, so
 // the order of issue (O += P V before the next S of the same tile) is all the synchronisation that the
-// reuse needs.  The running maximum moves only when it grows by more than 2^8 (the weights stay below
-// 256 in that case, exact in the sum and the same relative rounding in P), so the accumulator in TMEM
-// is rescaled rarely.
+// reuse needs.  The running maximum moves only when it grows by more than 2^kSlack (the weights stay below
+// that, exact in the sum and the same relative rounding in P), so the accumulator in TMEM is rescaled
+// rarely: 2^8, for fp16 2^3, which leaves the weights more of its range (kLift, as in the few-rows kernel).
 //
 // int8 pages: the codes are exact in 16 bits; S of each 64-dim block is a separate accumulator that the
 // softmax multiplies by the block's K scale in fp32, and P is multiplied by the V scale of each block
@@ -571,7 +571,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attention_tiles_paged(const
                 }
             }
             float m_ref = -INFINITY, l = 0.0f;
-            constexpr bool kUnits = I8 && std::is_same<T, __half>::value;
+            constexpr bool kHalf = std::is_same<T, __half>::value, kUnits = I8 && kHalf;
+            // log2 of how far a weight may pass 2^kLift, and of the weight at the maximum that m_ref was taken
+            // from: together below fp16's 65504 (int8: times a V scale over its unit, below 2)
+            constexpr float kSlack = kHalf ? 3.0f : 8.0f, kLift = !kHalf ? 0.0f : (I8 ? 11.0f : 12.0f);
             float unit[NH];
 #pragma unroll
             for (int b = 0; b < NH; ++b) unit[b] = 0.0f;
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attention_tiles_paged(const
                             if (!(m >> k & 1u)) s[32 * w + k] = -INFINITY;
                     }
                 }
-                // ---- running maximum: moved when it grows by more than 2^8 ----
+                // ---- running maximum: moved when it grows by more than 2^kSlack ----
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
                 for (int k = 4; k < BK; k += 8) {
@@ -640,9 +643,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) k_attention_tiles_paged(const
                     for (int j = 0; j < 4; ++j)
                         mx[j] = k + j + 4 < BK ? fmaxf(fmaxf(mx[j], s[k + j]), s[k + j + 4]) : fmaxf(mx[j], s[k + j]);
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+                const float top = fmaf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), a.scale_log2, -kLift);
                 float alpha = 1.0f;
-                const bool grow = top > m_ref + 8.0f || (m_ref == -INFINITY && top > -INFINITY);
+                const bool grow = top > m_ref + kSlack || (m_ref == -INFINITY && top > -INFINITY);
                 if (grow) {
                     alpha = m_ref == -INFINITY ? 0.0f : ex2(m_ref - top);
                     m_ref = top;

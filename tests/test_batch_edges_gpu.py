@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_batch_gpu import BF, I8, _batch, _check, _cu, _dense, _fast_reference, _gen, _plan_by_hand
+from test_batch_gpu import BF, FP, I8, _batch, _check, _cu, _dense, _fast_reference, _gen, _plan_by_hand, _want
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,45 @@ def test_attention_windows_of_any_size(kernels, m):
     for window, sinks in ((2**31 - 1, 0), (2**31 - 1, 2**31 - 1), (2**31 - 30, 5), (1, 2**31 - 1)):
         got = kernels.attention_paged(q, cache, table, lens_t, cu, window=window, sinks=sinks, return_lse=True)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), (window, sinks)
+
+
+def _far_apart(kernels, m, dtype, cache_dtype, dim, n, copies, outlier):
+    """`copies` requests (enough that none is split over CTAs) of m rows of ones on the same n keys: all scores 0 but
+    of key 5, 17.6 above them and with a value of 0, or (outlier) 60 below them and with values 2^21 times the others'."""
+    q, cache, table, lens_t, _, _ = _batch(kernels, [n], [m], 6, 2, dim, 64, dtype, cache_dtype, with_cu=True)
+    score = (-60.0 if outlier else 17.6) / (dim * dim**-0.5)
+    page, at = table[0, 0].long(), 5
+    cache.k.zero_()
+    if cache_dtype == I8:
+        cache.k[page, at] = 127 if score > 0 else -127
+        cache.k_scales.fill_(abs(score) / 127)
+        cache.v.copy_(cache.v.abs().clamp(min=1))
+        cache.v_scales.fill_(0.01)
+    else:
+        cache.k[page, at] = score
+        cache.v.copy_(cache.v.abs())
+    if outlier:
+        cache.v_scales[page, at] = 0.01 * 2**21
+    else:
+        cache.v[page, at] = 0
+    q.fill_(1.0)
+    scale = dim**-0.5
+    out, lse = kernels.attention_paged(q.repeat(copies, 1, 1), cache, table.expand(copies, -1), lens_t.expand(copies).contiguous(),
+                                       _cu(list(range(0, copies * m + 1, m))), scale=scale, return_lse=True)
+    want = tuple(x.repeat(copies, *(1,) * (x.dim() - 1)) for x in _want(q, cache, table, [n], [m], 64, 0, 0, scale))
+    _check(out, lse, want, dtype, str((m, dtype, cache_dtype, dim)))
+
+
+# few rows, and enough for the many-rows kernel
+@pytest.mark.parametrize("m,copies", [(1, 400), (5, 400), (40, 80)])
+@pytest.mark.parametrize("dtype,cache_dtype,dim", [(FP, FP, 64), (FP, FP, 128), (BF, I8, 128), (FP, I8, 64), (FP, I8, 128), (BF, BF, 64)])
+def test_attention_long_low_tail(kernels, m, copies, dtype, cache_dtype, dim):
+    """Weights 2^25 below the largest carry the output where the largest one's value is 0: they keep their bits."""
+    _far_apart(kernels, m, dtype, cache_dtype, dim, 30000, copies, False)
+
+
+@pytest.mark.parametrize("m,copies", [(1, 400), (5, 400), (40, 80)])
+@pytest.mark.parametrize("dtype,dim", [(BF, 128), (FP, 64), (FP, 128)])
+def test_attention_value_scale_far_above_the_others(kernels, m, copies, dtype, dim):
+    """An int8 key of no weight whose V scale is 2^21 times the others' does not cost them their bits."""
+    _far_apart(kernels, m, dtype, I8, dim, 700, copies, True)
