@@ -440,8 +440,9 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
             }
             q_scale[n][0] = q_scale[n][1] = a.scale_log2;
             if constexpr (!std::is_same<C, T>::value) {
-                // bf16 rows as fp16 times a power of two (the row's largest element in [1, 2)): exact, but for
-                // elements below 2^-14 of the largest, which lose less than 2^-25 of it
+                // bf16 rows as fp16 times a power of two that brings the row's largest element to [2^14, 2^15): exact
+                // for elements down to 2^-28 of the largest (smaller ones lose less than 2^-39 of it), so also where
+                // the largest meets codes of 0.  Rows all below 2^-100 are lifted as those.
                 float x[NQ][8], top = 0.0f;
 #pragma unroll
                 for (int i2 = 0; i2 < NQ; ++i2) {
@@ -452,14 +453,15 @@ __global__ void __launch_bounds__(RowsGeom<I8, D>::kThreads, RowsGeom<I8, D>::kC
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-                ex = top == 0.0f || ex > 127 ? 0 : min(ex, 126);
-                const float down = __int_as_float((127 - ex) << 23), up = __int_as_float((127 + max(ex, -126)) << 23);
+                ex = ex > 127 ? 0 : max(ex, -100) - 14;
+                const float down = __int_as_float((127 - ex) << 23), up = __int_as_float((127 + ex) << 23);
 #pragma unroll
                 for (int i2 = 0; i2 < NQ; ++i2)
                     qf[n][i2] = make_uint4(pack2<C>(x[i2][0] * down, x[i2][1] * down), pack2<C>(x[i2][2] * down, x[i2][3] * down),
                                            pack2<C>(x[i2][4] * down, x[i2][5] * down), pack2<C>(x[i2][6] * down, x[i2][7] * down));
 #pragma unroll
-                for (int e = 0; e < 2; ++e) q_scale[n][e] *= __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
+                for (int e = 0; e < 2; ++e)  // not 0, whose product with a masked score would be NaN
+                    q_scale[n][e] = fmaxf(q_scale[n][e] * __shfl_sync(0xffffffffu, up, (2 * c + e) * 4), 1.17549435e-38f);
             }
         }
         // accumulator element 2 k + e of every tile: row 2 c + e (+ 8 n), key (or dim) g of half k

@@ -179,3 +179,25 @@ def test_attention_long_low_tail(kernels, m, copies, dtype, cache_dtype, dim):
 def test_attention_value_scale_far_above_the_others(kernels, m, copies, dtype, dim):
     """An int8 key of no weight whose V scale is 2^21 times the others' does not cost them their bits."""
     _far_apart(kernels, m, dtype, I8, dim, 700, copies, True)
+
+
+@pytest.mark.parametrize("m", [1, 2, 40])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_query_elements_far_apart(kernels, m, dim):
+    """bf16 queries on int8 pages: elements 2^20 below the row's largest count when that one meets codes of 0."""
+    q, cache, table, lens_t, cu, _ = _batch(kernels, [300], [m], 6, 2, dim, 16, BF, I8, with_cu=True)
+    q[..., 3] = 2.0**20
+    cache.k[..., 3] = 0
+    out, lse = kernels.attention_paged(q, cache, table, lens_t, cu, return_lse=True)
+    _check(out, lse, _want(q, cache, table, [300], [m], 16, 0, 0, dim**-0.5), BF)
+
+
+@pytest.mark.parametrize("size", [2.0**-133, 2.0**-100, 2.0**-40, 2.0**60, 3e38])
+def test_attention_query_rows_of_any_size(kernels, size):
+    """bf16 query rows from subnormal to the largest on int8 pages: the scores are in proportion (scales of the keys make up
+    for the size where the product has room)."""
+    q, cache, table, lens_t, _, _ = _batch(kernels, [200], [1], 6, 2, 64, 16, BF, I8)
+    q = q.clamp(-1, 1) * size
+    cache.k_scales.copy_(cache.k_scales * min(1 / size, 2.0**100))
+    out, lse = kernels.attention_paged(q, cache, table, lens_t, return_lse=True)
+    _check(out, lse, _want(q, cache, table, [200], [1], 16, 0, 0, 1 / 8), BF)
