@@ -123,12 +123,14 @@ class BatchDecoder:
     def generate(self, prompts: list[list[int]], n_new: int, prefix: list[int] | None = None, repetition: float = 1.0,
                  frequency: float = 0.0, presence: float = 0.0, biases: dict[int, float] | None = None,
                  mask: torch.Tensor | None = None, logits_out: list | None = None) -> list[list[int]]:
-        """n_new greedy tokens after each prompt.  prefix: tokens that come before every prompt, held once;
-        mask: int32 [ceil(vocab / 32)] bits of the allowed ids; logits_out collects each step's processed
-        logits."""
+        """n_new greedy tokens after each prompt.  prefix: tokens that come before every prompt, held once
+        (every row sees all of it, so a decoder with a window refuses one); mask: int32 [ceil(vocab / 32)] bits
+        of the allowed ids; logits_out collects each step's processed logits."""
         n, vocab = len(prompts), self.config["vocab"]
         if not 0 < n <= self.max_requests or any(not p for p in prompts):
             raise ValueError(f"1 to {self.max_requests} prompts that are not empty")
+        if prefix and self.window > 0:
+            raise ValueError("a shared prefix is attended without a window: give the joined prompts, or a decoder of window 0")
         longest = max(map(len, prompts)) + n_new
         if longest + len(prefix or []) > self.config["max_seq"]:
             raise ValueError("prompt and new tokens exceed the model's positions")

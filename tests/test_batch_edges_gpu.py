@@ -201,3 +201,26 @@ def test_attention_query_rows_of_any_size(kernels, size):
     cache.k_scales.copy_(cache.k_scales * min(1 / size, 2.0**100))
     out, lse = kernels.attention_paged(q, cache, table, lens_t, return_lse=True)
     _check(out, lse, _want(q, cache, table, [200], [1], 16, 0, 0, 1 / 8), BF)
+
+
+# ---- the decoder of a batch -------------------------------------------------------------------------
+
+PROMPTS = [[5, 9, 100, 7, 3], [1], [400, 2, 2, 31, 8, 99, 17, 250, 40, 12, 13, 14, 15, 16, 18, 19, 20, 21]]
+
+
+@pytest.fixture(scope="module")
+def model(native):
+    from asdsl_b200.inference.synthetic import TINY, build_model
+
+    return build_model(TINY, 11)
+
+
+def test_prefix_with_a_window_is_refused(model):
+    """The shared prefix is attended whole by every row: under a window that would be another rule than without it."""
+    from asdsl_b200.inference.batch import BatchDecoder
+
+    dec = BatchDecoder(model, 4, 64, page_size=16, window=6, sinks=2)
+    with pytest.raises(ValueError, match="window"):
+        dec.generate(PROMPTS, 2, prefix=[3, 77, 500])
+    assert dec.taken == 0
+    assert len(dec.generate(PROMPTS, 2)[0]) == len(PROMPTS[0]) + 2
