@@ -123,8 +123,9 @@ class BatchDecoder:
     def generate(self, prompts: list[list[int]], n_new: int, prefix: list[int] | None = None, repetition: float = 1.0,
                  frequency: float = 0.0, presence: float = 0.0, biases: dict[int, float] | None = None,
                  mask: torch.Tensor | None = None, logits_out: list | None = None) -> list[list[int]]:
-        """n_new greedy tokens after each prompt.  prefix: tokens that come before every prompt, held once
-        (every row sees all of it, so a decoder with a window refuses one); mask: int32 [ceil(vocab / 32)] bits
+        """n_new greedy tokens after each prompt.  prefix: tokens that come before every prompt, held once and
+        part of each request's history for the penalties, not of what is returned (every row sees all of
+        it, so a decoder with a window refuses one); mask: int32 [ceil(vocab / 32)] bits
         of the allowed ids; logits_out collects each step's processed logits."""
         n, vocab = len(prompts), self.config["vocab"]
         if not 0 < n <= self.max_requests or any(not p for p in prompts):
@@ -132,7 +133,8 @@ class BatchDecoder:
         if prefix and self.window > 0:
             raise ValueError("a shared prefix is attended without a window: give the joined prompts, or a decoder of window 0")
         longest = max(map(len, prompts)) + n_new
-        if longest + len(prefix or []) > self.config["max_seq"]:
+        before = list(prefix or [])
+        if longest + len(before) > self.config["max_seq"]:
             raise ValueError("prompt and new tokens exceed the model's positions")
         shared = None
         if prefix:
@@ -140,10 +142,10 @@ class BatchDecoder:
             self._step(pre, [0], [len(prefix)], torch.tensor(prefix, dtype=torch.int32, device="cuda"), None)
             shared = (pre.block_table[0], len(prefix))
         plan = StepPlan(n, sum(map(len, prompts)), -(-longest // self.page_size), self.page_size)
-        history = torch.zeros(n, longest, dtype=torch.int32, device="cuda")
+        history = torch.zeros(n, len(before) + longest, dtype=torch.int32, device="cuda")
         for b, p in enumerate(prompts):
-            history[b, : len(p)] = torch.tensor(p, dtype=torch.int32)
-        prompt_lens = torch.tensor([len(p) for p in prompts], dtype=torch.int32, device="cuda")
+            history[b, : len(before) + len(p)] = torch.tensor(before + list(p), dtype=torch.int32)
+        prompt_lens = torch.tensor([len(before) + len(p) for p in prompts], dtype=torch.int32, device="cuda")
         ones = torch.ones(n, device="cuda")
         bias = {}
         if biases:
@@ -166,4 +168,4 @@ class BatchDecoder:
                 logits_out.append(logits)
             tokens = logits.argmax(-1).to(torch.int32)
             history.scatter_(1, lens.long()[:, None], tokens[:, None])
-        return [history[b, : len(p) + n_new].tolist() for b, p in enumerate(prompts)]
+        return [history[b, len(before) : len(before) + len(p) + n_new].tolist() for b, p in enumerate(prompts)]

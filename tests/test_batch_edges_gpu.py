@@ -224,3 +224,39 @@ def test_prefix_with_a_window_is_refused(model):
         dec.generate(PROMPTS, 2, prefix=[3, 77, 500])
     assert dec.taken == 0
     assert len(dec.generate(PROMPTS, 2)[0]) == len(PROMPTS[0]) + 2
+
+
+def test_penalties_see_the_prefix(model):
+    """The prefix's ids are part of each request's history, as if they stood in its prompt."""
+    from asdsl_b200.inference.batch import BatchDecoder
+
+    prefix = [3, 77, 500, 41, 6, 8]
+    dec = BatchDecoder(model, 4, 64, page_size=16)
+    plain, repeated, counted = [], [], []
+    dec.generate(PROMPTS, 1, prefix=prefix, logits_out=plain)
+    dec.reset()
+    dec.generate(PROMPTS, 1, prefix=prefix, repetition=8.0, logits_out=repeated)
+    dec.reset()
+    dec.generate(PROMPTS, 1, prefix=prefix, frequency=3.0, presence=5.0, logits_out=counted)
+    for b, p in enumerate(PROMPTS):
+        x, y = plain[0][b], repeated[0][b]
+        want = x.clone()
+        ids = torch.tensor(sorted(set(prefix + p)), device="cuda")
+        want[ids] = torch.where(x[ids] > 0, x[ids] / 8, x[ids] * 8)  # a power of two: exact
+        assert torch.equal(y, want)
+        assert torch.equal(counted[0][b], x)  # no output yet
+
+
+def test_penalties_under_a_prefix_as_over_the_joined_prompts(model):
+    """generate([p], prefix=P) and generate([P + p]) penalise the same ids and give the same logits (within the two
+    attentions' rounding, re-quantized to 8 bits by each projection: 5e-2 of the logits' norm)."""
+    from asdsl_b200.inference.batch import BatchDecoder
+
+    prefix = [3, 77, 500, 41, 6, 8, 7, 3]
+    dec = BatchDecoder(model, 4, 64, page_size=16)
+    shared, joined = [], []
+    dec.generate(PROMPTS, 1, prefix=prefix, repetition=8.0, logits_out=shared)
+    dec.reset()
+    dec.generate([prefix + p for p in PROMPTS], 1, repetition=8.0, logits_out=joined)
+    x, y = shared[0].double(), joined[0].double()
+    assert ((x - y).norm(dim=-1) <= 5e-2 * y.norm(dim=-1)).all()
