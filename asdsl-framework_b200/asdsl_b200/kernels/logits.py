@@ -23,7 +23,7 @@ def logits_process(logits: torch.Tensor, *, tokens: torch.Tensor | None = None, 
     * bit v % 32 of the int32 mask[b, v // 32] clear: -inf.
 
     Arithmetic in fp32, one rounding at the end.  Any part may be left out; ids outside the vocabulary
-    are ignored.  out may be `logits` itself.
+    are ignored.  out may be `logits` itself.  For inference: the result carries no gradient.
     """
     _not_cuda(logits, "logits")
     dtype, device, f32 = logits.dtype, logits.device, torch.float32

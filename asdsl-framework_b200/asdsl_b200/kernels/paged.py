@@ -12,7 +12,8 @@ document): those are attended once for the whole batch.
 
 All tensors are CUDA tensors on one device; calls enqueue work on torch's current stream of that
 device and do not synchronize.  Lengths and tables are read on the device, so a step can be captured
-in a CUDA graph.  There is no CPU path: without the library or a GPU the calls raise.
+in a CUDA graph.  There is no CPU path: without the library or a GPU the calls raise.  The operators
+are for inference: what they return carries no gradient, whatever the inputs require.
 """
 
 from __future__ import annotations
@@ -156,8 +157,8 @@ def plan_step(plan: StepPlan, kv_lens: torch.Tensor, new_lens: torch.Tensor, fre
 class PagedKV:
     """One layer's cache in pages: k and v [pages, page_size, kv_heads, head_dim].
 
-    bf16, fp16, or int8 codes with fp32 scales [pages, page_size, kv_heads, head_dim / 64] by the decode
-    engine's rule.  k and v may be strided alike (the halves of one tensor, heads before positions), with
+    bf16, fp16, or int8 codes with fp32 scales [pages, page_size, kv_heads, head_dim / 64], one for each
+    64 dims as in the decode engine's cache.  k and v may be strided alike (the halves of one tensor, heads before positions), with
     consecutive head_dim and strides of multiples of 16 bytes; scales are contiguous.
     """
 
@@ -204,9 +205,10 @@ class PagedKV:
 def kv_write(cache: PagedKV, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Write k and v [tokens, kv_heads, head_dim] to the cache's slots (``plan.slots``; -1 is skipped).
 
-    fp32, bf16 or fp16 into an int8 cache (quantized by the decode engine's rule), a 16-bit type or
-    fp32 into a cache of that 16-bit type.  Both may be strided alike, as columns of one projection.
-    A slot named twice in one call holds one of the two tokens.
+    fp32, bf16 or fp16 into an int8 cache, a 16-bit type or fp32 into a cache of that 16-bit type.  int8: per
+    64 dims the scale is max / 127 and the code the nearest multiple, with the decode engine's scales bit for
+    bit and its codes but where a value lies within 2^-22 of the boundary between two of them.  Both may be
+    strided alike, as columns of one projection.  A slot named twice in one call holds one of the two tokens.
     """
     _not_cuda(k, "k")
     dtype, device = k.dtype, cache.device
@@ -368,8 +370,11 @@ def attention_paged(q: torch.Tensor, cache: PagedKV, block_table: torch.Tensor, 
     them.  The i-th of n new tokens stands at p = kv_len - n + i and sees keys j <= p; with window > 0
     only those with j > p - window or j < sinks.  Returns out (of q's shape and type), or (out, lse)
     with return_lse: lse [tokens, heads] is the log of the sum of exp(scale * q . k).  A row that sees no
-    key gives 0 and -inf; a key whose table entry names no page is not seen.  Rows of q past cu_q[-1]
-    are not written.
+    key gives 0 and -inf; a key whose table entry names no page, or that lies past the table, is not seen
+    (positions come from kv_lens all the same).  Rows of q past cu_q[-1] are not written.  Softmax weights
+    take part in the second product as 16-bit numbers, for fp16 products (fp16 queries; int8 caches with few
+    rows) lifted by a power of two: all bits down to 2^-25 of the row's largest (int8: with each weight's V
+    scale over the largest one among the keys so far).
     """
     out, lse, scale = _attention_inputs(q, cache, block_table, kv_lens, cu_q, scale, out, lse, return_lse)
     if window < 0 or sinks < 0:

@@ -135,8 +135,8 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-// Four int8 codes as two fp16 pairs, exact: the byte c + 128 goes into the mantissa of 1024 + (c + 128),
-// and 1152 is subtracted.
+// Four int8 codes as two fp16 pairs, exact, by a known method: the byte c + 128 goes into the mantissa of
+// 1024 + (c + 128), and 1152 is subtracted.
 __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t& p01, uint32_t& p23) {
     const uint32_t u = w ^ 0x80808080u;
     const __half2 off = __half2half2(__ushort_as_half(0x6480));

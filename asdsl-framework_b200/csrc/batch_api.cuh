@@ -133,7 +133,7 @@ inline int launch_tiles(const AttnPagedArgs& a, long long grid, cudaStream_t st)
 constexpr int kMinTilesPerSplit = 4;
 constexpr int kManyKeys = 2048;  // from here 9 to 16 rows of a single request go to the many-rows kernel
 
-// Parts in scratch memory: `acc` of up to n + extra of them, then `ml`.
+// What a launch left in parts: where their maxima and sums lie (behind the outputs), and how many there are.
 struct AttnParts {
     float2* ml;
     int n;

@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 3) k_logits_touch(const Logits
         __syncthreads();
         if (!waited) grid_dependency_wait();
         waited = true;
-                for (int j0 = j_first; j0 < j_end; j0 += kSlots * j_step) {
+        for (int j0 = j_first; j0 < j_end; j0 += kSlots * j_step) {
             uint32_t w[kSlots], bits[kSlots];
             int v[kSlots];
 #pragma unroll

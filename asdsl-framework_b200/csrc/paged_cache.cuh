@@ -242,9 +242,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // One thread per 8 dims of a (token, head), K and V both: 16-byte loads and stores (8-byte code
-// stores for int8).  The int8 rule is the decode engine's: per 64 dims (8 threads) scale = amax *
-// fl(1/127), code = rne(x * inv) clamped to +-127, scale 1e-12 for a block of zeros; inv = 127 / amax is
-// rounded twice here and once there, so a code within a last bit of a rounding boundary can differ by a step.
+// stores for int8).  int8: per 64 dims (8 threads) scale = amax * fl(1/127), code = rne(x * inv) clamped to
+// +-127, scale 1e-12 for a block of zeros.  The scales are the decode engine's bit for bit; inv is 127 * (1 /
+// amax), rounded twice, where the engine rounds 127 / amax once, so a value within 2^-22 of a rounding boundary can
+// have the neighbouring code (1.3e-6 of fp32 values; of bf16 ones 3.2e-4, all exact ties).  The values held
+// are as near either way (relative error 0.0059301 of normal values, at most 0.50001 steps).
+// Bound by memory: 16384 tokens x 8 x 128 bf16 24.6 us (5.5 TB/s), fp32 -> int8 30.9, bf16 -> int8 24.6.
 template <typename SRC, typename DST>
 __global__ void __launch_bounds__(256) k_kv_write(const KvWriteArgs a) {
     const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;

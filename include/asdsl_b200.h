@@ -560,7 +560,8 @@ int asdsl_b200_plan_step(const int32_t* kv_lens, const int32_t* new_lens, int n_
 /* Writes k and v [n_tokens][kv_heads][head_dim] (fp32, bf16 or fp16; strides in elements) to the slots;
  * a slot outside the cache is skipped.  A 16-bit cache takes its own type or fp32 (rounded to nearest
  * even); an int8 cache quantizes each 64 dims as the engine's set_kv_cache does
- * (unified_engine.cpp:872-917), with 127 / amax computed as 127 * (1 / amax). */
+ * (unified_engine.cpp:872-917), with 127 / amax computed as 127 * (1 / amax): the same scales, and the same
+ * codes but for values within 2^-22 of a rounding boundary. */
 int asdsl_b200_kv_write(const asdsl_b200_paged_cache* cache, const void* k, const void* v, int dtype,
                         long long token_stride, long long head_stride, const int32_t* slots, int n_tokens, void* stream);
 
@@ -574,7 +575,7 @@ size_t asdsl_b200_attention_workspace_bytes(int n_requests, int n_tokens, int he
  * kv_len - n + i and sees keys j <= p with, when window > 0, j > p - window or j < sinks.  out
  * [n_tokens][heads][head_dim] contiguous, the type of q; lse (may be NULL) [n_tokens][heads] the natural
  * log of the sum of exp(scale * q . k).  A row that sees no key gives 0 and -inf.  Keys whose table entry
- * is not a page of the cache count as unseen.  Rows of q past cu_q[n_requests] are left alone. */
+ * is not a page of the cache, or that lie past table_width, count as unseen.  Rows of q past cu_q[n_requests] are left alone. */
 int asdsl_b200_attention_paged(const void* q, int q_dtype, long long q_token_stride, long long q_head_stride,
                                const asdsl_b200_paged_cache* cache, const int32_t* block_table, long long table_stride,
                                int table_width, const int32_t* kv_lens, const int32_t* cu_q, int n_requests, int n_tokens,
