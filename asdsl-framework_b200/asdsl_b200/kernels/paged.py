@@ -97,7 +97,8 @@ class StepPlan:
     last), ``counts`` = (pages taken, new tokens, flags).
 
     ``total_lens`` may be the next step's kv_lens: a step that reads it writes its totals to another buffer,
-    which ``total_lens`` then names.
+    which ``total_lens`` then names.  (A captured step replays with the buffers of its capture: give it lengths
+    in a buffer of the caller's.)
     """
 
     FREE_SHORT, TABLE_NARROW, TOKENS_OVER = 1, 2, 4  # counts[2]
